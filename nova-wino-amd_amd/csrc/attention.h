@@ -461,6 +461,11 @@ inline float score_scale(const Attention& a) {
     return a.scale != 0 ? (a.scale < 0 ? -a.scale : a.scale) * 1.44269504088896341f : 1.0f;
 }
 
+// Where the running maximum of a row's scores starts: it stays finite times
+// c = score_scale, so that a row (or the keys of it so far) without any score
+// above -inf has exponentials of 0 and a sum of 0, not NaN.
+inline float lowest_score(float c) { return -0x1p127f / (c > 1.0f ? c : 1.0f); }
+
 inline bool close_rows(int64_t stride) { return stride >= 0 && stride < (1 << 23); }
 
 }  // namespace nova

@@ -43,7 +43,7 @@ struct FwdArgs {
     int qvec, kvec, vvec;  // rows in 16-byte chunks
     // The scores are c q . k, c > 0: the scale's sign goes into the queries
     // (flip: their sign bits), and a scale of 0 makes them zeros (live: 0).
-    float c;
+    float c, lowest;  // lowest: see lowest_score
     unsigned flip, live;
 };
 
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(DV)) void attention_kernel
     f16v o[DV];
 #pragma unroll
     for (int d = 0; d < DV; d++) o[d] = f16v{};
-    float m = -3.402823466e38f, l = 0.0f;  // the row's maximum; this lane's part of its sum
+    float m = a.lowest, l = 0.0f;  // the row's maximum; this lane's part of its sum
 
     KeyTiles tiles(split * a.per,
                    min((a.Lk + kKeyTile - 1) / kKeyTile, split * a.per + a.per), a.Lk,
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kPairThreads, 2) void attention_pair_kernel(FwdArgs
     f16v o[DV];
 #pragma unroll
     for (int d = 0; d < DV; d++) o[d] = f16v{};
-    float m = -3.402823466e38f, l = 0.0f;
+    float m = a.lowest, l = 0.0f;
     KeyTiles tiles(split * a.per,
                    min((a.Lk + kKeyTile - 1) / kKeyTile, split * a.per + a.per), a.Lk,
                    a.mask ? a.mask + b * a.mask_stride : nullptr, bits, 2 * kWaves);
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(kThreads) void attention_few_kernel(FwdArgs a) {
     float q[R][8], o[R][8], m[R], l[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        m[r] = -3.402823466e38f;
+        m[r] = a.lowest;
         l[r] = 0.0f;
         u4 x = {0, 0, 0, 0};
         if (r < rows) {
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(kThreads) void attention_few_kernel(FwdArgs a) {
     __shared__ float so[kWaves][R][8 * LPK], sm[kWaves][R], sl[kWaves][R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        float mn = l[r] > 0.0f || l[r] != l[r] ? m[r] : -3.402823466e38f;
+        float mn = l[r] > 0.0f || l[r] != l[r] ? m[r] : a.lowest;
 #pragma unroll
         for (int w = LPK; w < 64; w *= 2) mn = fmaxf(mn, __shfl_xor(mn, w));
         const float f = l[r] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((m[r] - mn) * a.c);
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(kThreads) void attention_few_kernel(FwdArgs a) {
     for (int i = tid; i < rows * 8 * LPK; i += kThreads) {
         const int r = i / (8 * LPK), e = i % (8 * LPK);
         if (e >= a.D) continue;
-        float mn = -3.402823466e38f, sum = 0.0f, x = 0.0f;
+        float mn = a.lowest, sum = 0.0f, x = 0.0f;
         for (int w = 0; w < kWaves; w++)
             if (sl[w][r] != 0.0f) mn = fmaxf(mn, sm[w][r]);
         for (int w = 0; w < kWaves; w++)
@@ -743,6 +743,7 @@ hipError_t launch_attention(const Attention& a, const AttentionPlan& plan, uint1
     f.kvec = chunked(a.k, a.ks, a.D) && close_rows(a.ks[1]);
     f.vvec = chunked(a.v, a.vs, a.D) && close_rows(a.vs[1]);
     f.c = score_scale(a);
+    f.lowest = lowest_score(f.c);
     f.flip = a.scale < 0 ? 0x80008000u : 0u;
     f.live = a.scale != 0 ? ~0u : 0u;
     if (plan.splits > 1) {

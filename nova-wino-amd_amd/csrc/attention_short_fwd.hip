@@ -26,7 +26,7 @@ struct ShortArgs {
     int B, Bk, Lq, Lk, H, group, D;
     int blocks, per, n;  // workgroups of a head; blocks of 32 rows for each wave; workgroups
     int qvec, kvec, vvec;
-    float c;
+    float c, lowest;  // lowest: see lowest_score
     unsigned flip, live;
 };
 
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(kThreads, short_waves(16 * DK)) void attention_shor
 #pragma unroll
         for (int s = 0; s < DK; s++) qf[s] = (qf[s] & a.live) ^ a.flip;
         f16v s[NB];
-        float m = -3.402823466e38f;
+        float m = a.lowest;
 #pragma unroll
         for (int kb = 0; kb < NB; kb++) {
             s[kb] = start_scores(bias + 32 * kb, half);
@@ -169,6 +169,7 @@ hipError_t launch_attention_short(const Attention& a, int per, uint16_t* out, ui
     f.kvec = chunked(a.k, a.ks, a.D);
     f.vvec = chunked(a.v, a.vs, a.D);
     f.c = score_scale(a);
+    f.lowest = lowest_score(f.c);
     f.flip = a.scale < 0 ? 0x80008000u : 0u;
     f.live = a.scale != 0 ? ~0u : 0u;
     return a.bf16 ? launch_all<BF16>(f, s) : launch_all<F16>(f, s);
