@@ -83,6 +83,7 @@ struct GnArgs {
     int grid;         // workgroups of the launch that writes dx, without params_done's
     int sets;         // channels-last, one launch: workgroups of an image
     int share;        // channels-last: lanes that add up one group's values
+    int span;         // channels-last: groups that the workgroup adds up at a time
     int cols;         // channels-last: vectors per pixel that a workgroup owns
     Div width;        // channels of a group
     Div across;       // channels-last: a group's values in a row of threads
@@ -367,8 +368,8 @@ struct Spot {
 // of each group; out[g] (LDS) holds fin(total, g) for each of the workgroup's
 // `groups` groups. red: bands * cols * V floats. Inactive threads bring zeros. A
 // group's values are shared by up to 64 neighbouring lanes, so no thread walks
-// a long column of them alone.
-template <int V, typename F>
+// a long column of them alone. MANY: groups may outnumber the threads.
+template <int V, bool MANY, typename F>
 __device__ __forceinline__ void group_totals(float (&v)[V], const Spot& at, const GnArgs& a,
                                              int groups, float* red, float* out, F fin) {
     const bool single = a.across.d < a.n || V == 1;  // a thread's channels are of one group
@@ -388,8 +389,8 @@ __device__ __forceinline__ void group_totals(float (&v)[V], const Spot& at, cons
     }
     __syncthreads();
     const int lanes = a.share, per = a.across.d, bands = a.bands();
-    const int g = threadIdx.x / lanes, l = threadIdx.x & (lanes - 1);
-    if (g < groups) {
+    const int l = threadIdx.x & (lanes - 1);
+    for (int g = threadIdx.x / lanes; g < groups; g += a.span) {
         float s = 0.0f;
         int r = a.across.quot(l), c = l - r * per;
         const int dr = a.across.quot(lanes), dc = lanes - dr * per;
@@ -404,6 +405,7 @@ __device__ __forceinline__ void group_totals(float (&v)[V], const Spot& at, cons
         }
         s = sum_lanes(s, lanes);
         if (l == 0) out[g] = fin(s, g);
+        if (!MANY) break;
     }
     __syncthreads();
 }
@@ -442,7 +444,7 @@ __global__ __launch_bounds__(TH) void norm_nhwc_one_kernel(GnArgs a) {
     }
     const float count = (float)a.n * (float)a.P, part = 1.0f / count;
     const int64_t at = (int64_t)b * a.G + g0;
-    group_totals<V>(s, spot, a, groups, red, total, [&](float t, int g) {
+    group_totals<V, false>(s, spot, a, groups, red, total, [&](float t, int g) {
         const float m = t * part;
         a.mean[at + g] = m;
         return m;
@@ -459,7 +461,7 @@ __global__ __launch_bounds__(TH) void norm_nhwc_one_kernel(GnArgs a) {
                 s[j] = __builtin_fmaf(d, d, s[j]);
             }
     }
-    group_totals<V>(s, spot, a, groups, red, total, [&](float t, int g) {
+    group_totals<V, false>(s, spot, a, groups, red, total, [&](float t, int g) {
         const float r = rstd_of(t, count, a.eps);
         a.rstd[at + g] = r;
         return r;
@@ -503,7 +505,7 @@ struct Place {
 
 // Statistics of a piece's groups. A thread keeps a running mean and squared
 // deviations of each of its channels, kStream pixels at a time.
-template <typename T, int V>
+template <typename T, int V, bool MANY>
 __global__ __launch_bounds__(kWide) void stats_nhwc_kernel(GnArgs a) {
     extern __shared__ float lds[];  // bands * C, then G
     float *red = lds, *total = lds + a.bands() * a.C;
@@ -548,7 +550,7 @@ __global__ __launch_bounds__(kWide) void stats_nhwc_kernel(GnArgs a) {
     for (int j = 0; j < V; j++) s[j] = m[j] * n;
     const float count = (float)a.n * (float)(at.p1 - at.p0), part = 1.0f / count;
     float* to = a.part + 3 * ((int64_t)at.b * a.G * a.pieces + at.piece);
-    group_totals<V>(s, at.spot, a, a.G, red, total, [&](float t, int g) {
+    group_totals<V, MANY>(s, at.spot, a, a.G, red, total, [&](float t, int g) {
         const float mean = t * part;
         to[3 * (int64_t)g * a.pieces] = count;
         to[3 * (int64_t)g * a.pieces + 1] = mean;
@@ -564,7 +566,7 @@ __global__ __launch_bounds__(kWide) void stats_nhwc_kernel(GnArgs a) {
         const float d = m[j] - total[g];
         s[j] = __builtin_fmaf(d * d, n, q[j]);
     }
-    group_totals<V>(s, at.spot, a, a.G, red, total, [&](float t, int g) {
+    group_totals<V, MANY>(s, at.spot, a, a.G, red, total, [&](float t, int g) {
         to[3 * (int64_t)g * a.pieces + 2] = t;
         return t;
     });
@@ -1228,7 +1230,7 @@ void place(Plan* p, int width, int groups) {
     p->rows = 64 / p->lanes_c * (p->TH / 64 / p->tiles);
     p->across = width % p->V == 0 ? width / p->V : width;
     p->share = 64;
-    while (p->share * groups > p->TH) p->share /= 2;
+    while (p->share > 1 && p->share * groups > p->TH) p->share /= 2;
 }
 
 Plan plan_of(const GroupNorm& g, const void* const* ptrs, int n, bool backward, int cus) {
@@ -1269,7 +1271,8 @@ Plan plan_of(const GroupNorm& g, const void* const* ptrs, int n, bool backward, 
         p.tiles = (int)div_up(nv, p.lanes_c);
         auto waves = [&](int some) {
             int bands = std::max(1, some / p.tiles);
-            while (64 * p.tiles * bands < g.G) bands++;
+            // a thread for every group, where a workgroup holds that many
+            while (64 * p.tiles * bands < g.G && 64 * p.tiles * (bands + 1) <= kWide) bands++;
             p.TH = 64 * p.tiles * bands;
             place(&p, width, g.G);
         };
@@ -1343,6 +1346,7 @@ GnArgs args_of(const GroupNorm& g, const Plan& p) {
     a.grid = (int)p.grid;
     a.sets = p.sets;
     a.share = p.share;
+    a.span = p.share > 0 ? p.TH / p.share : 0;
     a.cols = p.cols;
     a.lanes_c = p.lanes_c;
     a.tiles = p.tiles;
@@ -1382,7 +1386,9 @@ void forward_v(const GroupNorm& g, const Plan& p, const GnArgs& a, hipStream_t s
     }
     const dim3 grid((unsigned)p.grid), block(p.TH), groups((unsigned)(g.B * g.G));
     if (g.nhwc) {
-        launch_lds(stats_nhwc_kernel<T, V>, grid, block, 4 * (a.bands() * a.C + a.G), s, a);
+        const size_t lds = 4 * ((size_t)a.bands() * a.C + a.G);
+        if (a.G > p.TH) launch_lds(stats_nhwc_kernel<T, V, true>, grid, block, lds, s, a);
+        else launch_lds(stats_nhwc_kernel<T, V, false>, grid, block, lds, s, a);
         if (p.join) {
             launch(norm_join_kernel, groups, dim3(64), s, a, p.pieces);
             launch(apply_nhwc_kernel<T, V, false>, grid, block, s, a);

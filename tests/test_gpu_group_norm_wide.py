@@ -1,0 +1,30 @@
+"""nova_group_norm with more groups than a workgroup of its layout's width has
+threads: three to seven channels a group above 2048 channels, channels-last. The
+definition in float64 and its tolerances are test_gpu_group_norm.py's."""
+
+import pytest
+import torch
+
+from test_gpu_group_norm import _case, _check
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [  # B, C, G, H, W
+    (2, 2304, 768, 5, 5),     # forward in one launch
+    (1, 2304, 768, 46, 47),   # forward in pieces
+    (1, 2064, 688, 3, 7),
+    (1, 4608, 768, 30, 21),
+    (2, 5120, 1024, 9, 4),
+    (1, 7168, 1024, 24, 25),
+    (1, 8192, 1024, 5, 3),    # the most channels and groups
+    (1, 2304, 576, 46, 47),   # as many groups as threads
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_more_groups_than_threads(shape, dtype):
+    B, C, G, H, W = shape
+    print(f"[group norm] {shape} {dtype}", flush=True)
+    x, w, b, gy = _case(B, C, H, W, dtype, True, seed=C)
+    _check(x, G, w, b, gy, silu=C % 5 != 0)
