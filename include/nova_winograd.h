@@ -260,7 +260,9 @@ NOVA_API const char* nova_profile_kernel_name(nova_handle_t h, int kind);
 
 /* x: [batch][channels][pixels], or [batch][pixels][channels] with
  * channels_last = 1; dense. weight, bias: `channels` values of param_dtype,
- * each may be NULL (1 and 0). */
+ * each may be NULL (1 and 0). Refused beside bad arguments: calls with a launch
+ * of 2^32 threads or more (256 for every image and group, mostly), more than
+ * 2^40 values or more than 2^31 - 2^20 - 1 pixels. */
 typedef struct {
     const void *x, *weight, *bias;
     int dtype, param_dtype;

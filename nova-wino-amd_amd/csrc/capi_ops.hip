@@ -75,7 +75,8 @@ bool group_norm_args(const char* fn, const nova_group_norm_t* p, GroupNorm* g) {
         return false;
     }
     const int64_t n = times(times(p->batch, p->channels), p->pixels);
-    if (n < 0 || n > (INT64_C(1) << 40) || p->pixels > INT_MAX ||
+    // the kernels' walks over an image's pixels step past its end by less than 2^20
+    if (n < 0 || n > (INT64_C(1) << 40) || p->pixels > INT_MAX - (1 << 20) ||
         (int64_t)p->batch * p->groups > (1 << 30) || (int64_t)p->batch * p->channels > (1 << 30)) {
         set_error(kErrInvalidArgument, "%s: shape exceeds launch limits", fn);
         return false;
@@ -88,6 +89,16 @@ bool group_norm_args(const char* fn, const nova_group_norm_t* p, GroupNorm* g) {
     *g = GroupNorm{p->x,     p->weight, p->bias,          p->dtype, p->param_dtype, p->batch,
                    p->channels, p->groups, p->pixels, p->channels_last, p->silu, p->eps};
     return true;
+}
+
+// Whether every launch of the call has fewer than 2^32 threads, which is what a
+// grid takes. Below 2^21 images times channels none comes near that many.
+bool group_norm_fits(const char* fn, const GroupNorm& g, bool backward, int cus) {
+    if ((int64_t)g.B * g.C < (1 << 21) ||
+        group_norm_launch(g, backward, cus).threads < (INT64_C(1) << 32))
+        return true;
+    set_error(kErrInvalidArgument, "%s: shape exceeds launch limits", fn);
+    return false;
 }
 
 bool attention_args(const char* fn, const nova_attention_t* p, Attention* a) {
@@ -163,8 +174,10 @@ extern "C" {
 
 long long nova_group_norm_workspace_bytes(const nova_group_norm_t* p, int backward) {
     GroupNorm g;
-    if (!group_norm_args("nova_group_norm_workspace_bytes", p, &g)) return -1;
+    const char* fn = "nova_group_norm_workspace_bytes";
+    if (!group_norm_args(fn, p, &g)) return -1;
     const int cus = compute_units();
+    if (!group_norm_fits(fn, g, backward != 0, cus)) return -1;
     return backward ? group_norm_bwd_ws(g, cus) : group_norm_ws(g, cus);
 }
 
@@ -183,6 +196,7 @@ void nova_group_norm(const nova_group_norm_t* p, void* d_y, float* d_mean, float
         return;
     }
     const int cus = compute_units();
+    if (!group_norm_fits(fn, g, false, cus)) return;
     if (!workspace_ok(fn, d_workspace, workspace_bytes, group_norm_ws(g, cus))) return;
     hip_ok(launch_group_norm(g, d_y, d_mean, d_rstd, d_workspace, cus,
                              static_cast<hipStream_t>(stream)),
@@ -212,6 +226,7 @@ void nova_group_norm_backward(const nova_group_norm_t* p, const void* d_grad_y,
         return;
     }
     const int cus = compute_units();
+    if (!group_norm_fits(fn, g, true, cus)) return;
     if (!none &&
         !workspace_ok(fn, d_workspace, workspace_bytes, group_norm_bwd_ws(g, cus)))
         return;

@@ -1173,17 +1173,19 @@ __global__ __launch_bounds__(kThreads) void sums_plain_kernel(GnArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void dx_plain_kernel(GnArgs a) {
     if (params_done(a, a.grid)) return;
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= (int64_t)a.B * a.C * a.P) return;
-    const int64_t pixel = a.nhwc ? i / a.C : i / a.P;  // (b, p), or (b, c)
-    const int c = (int)(a.nhwc ? i % a.C : pixel % a.C);
-    const int64_t b = a.nhwc ? pixel / a.P : pixel / a.C, g = b * a.G + c / a.n;
-    const float rstd = a.rstd[g], w = param(a.gamma, a.params, c, 1.0f);
-    const float xh = ((float)static_cast<const T*>(a.x)[i] - a.mean[g]) * rstd;
-    const float z = grad_z(xh, w, param(a.beta, a.params, c, 0.0f),
-                           (float)static_cast<const T*>(a.dy)[i], a.silu);
-    static_cast<T*>(a.y)[i] =
-        (T)(rstd * (__builtin_fmaf(w, z, -a.sums[2 * g]) - xh * a.sums[2 * g + 1]));
+    const int64_t all = (int64_t)a.B * a.C * a.P;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all;
+         i += (int64_t)a.grid * kThreads) {
+        const int64_t pixel = a.nhwc ? i / a.C : i / a.P;  // (b, p), or (b, c)
+        const int c = (int)(a.nhwc ? i % a.C : pixel % a.C);
+        const int64_t b = a.nhwc ? pixel / a.P : pixel / a.C, g = b * a.G + c / a.n;
+        const float rstd = a.rstd[g], w = param(a.gamma, a.params, c, 1.0f);
+        const float xh = ((float)static_cast<const T*>(a.x)[i] - a.mean[g]) * rstd;
+        const float z = grad_z(xh, w, param(a.beta, a.params, c, 0.0f),
+                               (float)static_cast<const T*>(a.dy)[i], a.silu);
+        static_cast<T*>(a.y)[i] =
+            (T)(rstd * (__builtin_fmaf(w, z, -a.sums[2 * g]) - xh * a.sums[2 * g + 1]));
+    }
 }
 
 // ---- choice of the form ----------------------------------------------------
@@ -1325,6 +1327,14 @@ Plan plan_of(const GroupNorm& g, const void* const* ptrs, int n, bool backward, 
     return p;
 }
 
+// Workgroups of dx_plain_kernel, whose threads walk further than their own
+// element where the tensor has more than that many.
+int plain_grid(const GroupNorm& g) {
+    return (int)std::min<int64_t>(div_up((int64_t)g.B * g.C * g.P, kThreads), 1 << 20);
+}
+
+int extra_of(const GroupNorm& g) { return (int)div_up(g.C, kParamChannels); }
+
 GnArgs args_of(const GroupNorm& g, const Plan& p) {
     GnArgs a{};
     a.x = g.x;
@@ -1463,6 +1473,26 @@ __global__ __launch_bounds__(kThreads) void zero_params_kernel(GnArgs a) {
 
 // The vector length, and with it the pieces, follows the alignment of the
 // call's tensors; the sizes below cover every alignment.
+GroupNormLaunch group_norm_launch(const GroupNorm& g, bool backward, int cus) {
+    GroupNormLaunch most{0, 0};
+    if (g.B == 0 || g.P == 0) return most;
+    auto add = [&](int64_t grid, int block) {
+        most.threads = std::max(most.threads, grid * block);
+        most.block = std::max(most.block, block);
+    };
+    for (uintptr_t align = 16; align >= 2; align /= 2) {
+        const void* at = reinterpret_cast<const void*>(align);
+        const Plan p = plan_of(g, &at, 1, backward, cus);
+        const int64_t groups = (int64_t)g.B * g.G;
+        if (p.form != kPlain) add(p.grid + (backward ? extra_of(g) : 0), p.TH);
+        else if (backward) add(std::max<int64_t>((int64_t)g.B * g.C, plain_grid(g) + extra_of(g)),
+                               kThreads);
+        if (backward || p.form == kPlain) add(groups, kThreads);
+        else if (p.join) add(groups, 64);
+    }
+    return most;
+}
+
 int64_t group_norm_ws(const GroupNorm& g, int cus) {
     int64_t most = 0;
     if (g.B == 0 || g.P == 0) return 0;
@@ -1520,10 +1550,10 @@ hipError_t launch_group_norm_bwd(const GroupNorm& g, const void* dy, const float
                    a);
         return hipGetLastError();
     }
-    if (p.form == kPlain) a.grid = (int)div_up((int64_t)g.B * g.C * g.P, kThreads);
+    if (p.form == kPlain) a.grid = plain_grid(g);
     a.sums = static_cast<float*>(ws);
     a.part = a.sums + 2 * (int64_t)g.B * g.G;
-    const int extra = dgamma != nullptr ? (int)div_up(g.C, kParamChannels) : 0;
+    const int extra = dgamma != nullptr ? extra_of(g) : 0;
     if (g.dtype == kF16) backward_t<_Float16>(g, p, a, extra, s);
     else if (g.dtype == kBF16) backward_t<__bf16>(g, p, a, extra, s);
     else backward_t<float>(g, p, a, extra, s);

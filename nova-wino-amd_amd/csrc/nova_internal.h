@@ -411,6 +411,12 @@ struct GroupNorm {
     int nhwc, silu;
     float eps;
 };
+// The largest launch of a call: threads of its grid, of its workgroup.
+struct GroupNormLaunch {
+    int64_t threads;
+    int block;
+};
+GroupNormLaunch group_norm_launch(const GroupNorm& g, bool backward, int cus);
 int64_t group_norm_ws(const GroupNorm& g, int cus);
 // mean, rstd: [B][G].
 hipError_t launch_group_norm(const GroupNorm& g, void* y, float* mean, float* rstd, void* ws,

@@ -28,3 +28,22 @@ def test_more_groups_than_threads(shape, dtype):
     print(f"[group norm] {shape} {dtype}", flush=True)
     x, w, b, gy = _case(B, C, H, W, dtype, True, seed=C)
     _check(x, G, w, b, gy, silu=C % 5 != 0)
+
+
+def test_more_elements_than_the_plain_grid():
+    """Two images of 2^27 elements and more each: the element-by-element form's
+    gradient walks further than its grid, and gives each image what it gives it
+    alone."""
+    from nova_winograd import nova_group_norm
+
+    C, H, W = 16384, 82, 100
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, gy = (torch.randn(2, H, W, C, generator=g, device="cuda", dtype=torch.float16)
+             .permute(0, 3, 1, 2) for _ in "xg")
+    both = x.detach().requires_grad_()
+    nova_group_norm(both, 32, activation="silu").backward(gy)
+    for i in range(2):
+        one = x[i:i + 1].detach().requires_grad_()
+        nova_group_norm(one, 32, activation="silu").backward(gy[i:i + 1])
+        assert torch.equal(one.grad, both.grad[i:i + 1])
+        assert one.grad.count_nonzero() > 0.9 * one.numel()
