@@ -293,7 +293,9 @@ NOVA_API void nova_group_norm_backward(const nova_group_norm_t* args, const void
  * dense. kv_batch is batch, or 1 where one sequence of keys serves them all;
  * query head h reads key head h / (heads / kv_heads). key_mask: bytes, 0 = the
  * key takes no part (its key and value may hold anything), sequence b's `keys`
- * bytes at key_mask + b * mask_stride; or NULL. head_dim: 1 to 256. */
+ * bytes at key_mask + b * mask_stride; or NULL. head_dim: 1 to 256. Refused beside
+ * bad arguments: batch * heads or kv_batch * kv_heads from 2^24 on, more than 2^28
+ * queries or keys, 2^29 rows over batch and heads, 2^36 values. */
 typedef struct {
     const void *q, *k, *v;
     const unsigned char* key_mask;

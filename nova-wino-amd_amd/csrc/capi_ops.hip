@@ -119,12 +119,16 @@ bool attention_args(const char* fn, const nova_attention_t* p, Attention* a) {
                   p->head_dim);
         return false;
     }
+    // A head of a sequence takes a workgroup of 256 threads, or one for each 128
+    // of its rows (or keys): fewer than 2^24 heads in all, and 2^29 rows, keep
+    // every launch below 2^32 threads.
     const int64_t rows = times(times(p->batch, p->heads), p->queries);
     const int64_t keys = times(times(p->kv_batch, p->kv_heads), p->keys);
     if (rows < 0 || keys < 0 || times(rows, p->head_dim) > (INT64_C(1) << 36) ||
         times(keys, p->head_dim) > (INT64_C(1) << 36) || rows > (1 << 29) || keys > (1 << 29) ||
         p->queries > (1 << 28) || p->keys > (1 << 28) ||
-        (int64_t)p->batch * p->heads > (1 << 24)) {
+        (int64_t)p->batch * p->heads >= (1 << 24) ||
+        (int64_t)p->kv_batch * p->kv_heads >= (1 << 24)) {
         set_error(kErrInvalidArgument, "%s: shape exceeds launch limits", fn);
         return false;
     }
