@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/python.h>
 
+#include <limits>
+
 #include "../../include/nova_winograd.h"
 
 namespace {
@@ -37,6 +39,13 @@ void* stream_of(const Tensor& t) {
 
 int dtype_code(at::ScalarType t) {
     return t == at::kHalf ? 0 : t == at::kBFloat16 ? 1 : t == at::kFloat ? 2 : -1;
+}
+
+// The C structures hold sizes as int.
+void require_ints(const char* fn, const char* name, at::IntArrayRef sizes) {
+    for (const int64_t n : sizes)
+        TORCH_CHECK_VALUE(n <= std::numeric_limits<int>::max(), fn, ": ", name, " of ", sizes,
+                          " exceeds launch limits");
 }
 
 // Scratch memory for one call from PyTorch's allocator: its owner may go when
@@ -183,6 +192,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const std::optional<Tensor>& 
                      x.scalar_type(), "; float16, bfloat16 and float32 are supported");
     TORCH_CHECK_VALUE(x.dim() >= 2, "nova_group_norm: input needs a batch and a channel axis");
     const int64_t C = x.size(1);
+    require_ints("nova_group_norm", "input", x.sizes().slice(0, 2));
     TORCH_CHECK_VALUE(groups >= 1 && C >= 1 && C % groups == 0, "nova_group_norm: num_groups (",
                       groups, ") does not divide the ", C, " channels");
     Tensor p[2] = {weight_.value_or(Tensor()), bias_.value_or(Tensor())};
@@ -303,6 +313,7 @@ Tensor cross_attention(const Tensor& query, const Tensor& key, const Tensor& val
         TORCH_CHECK_VALUE(t.dim() == 4 && t.device() == query.device(), "nova_cross_attention: ",
                           names[i], " has to be [batch, length, heads, channels] on ",
                           query.device(), ", got ", t.sizes(), " on ", t.device());
+        require_ints("nova_cross_attention", names[i], t.sizes());
     }
     const int64_t B = query.size(0), H = query.size(2), D = query.size(3);
     TORCH_CHECK_VALUE(key.sizes() == value.sizes() && (key.size(0) == B || key.size(0) == 1) &&
