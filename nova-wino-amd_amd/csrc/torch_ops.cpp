@@ -63,6 +63,20 @@ std::optional<Tensor> given(const Tensor& t) {
     return t.defined() ? std::optional<Tensor>(t) : std::nullopt;
 }
 
+// Whether a result takes part in a backward. Forward-mode derivatives are an
+// error: outside of the autograd functions nothing else would stop a tangent
+// from being dropped.
+bool recorded(const char* fn, std::initializer_list<const Tensor*> in) {
+    bool any = false;
+    for (const Tensor* t : in) {
+        if (!t->defined()) continue;
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), fn,
+                                    ": forward-mode derivatives are not implemented");
+        any |= t->requires_grad();
+    }
+    return any && at::GradMode::is_enabled();
+}
+
 // Gradients of a backward that runs with gradients enabled (create_graph): what
 // the kernels wrote cannot be differentiated again, which is an error only if
 // someone does.
@@ -207,9 +221,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const std::optional<Tensor>& 
         p[i] = p[i].contiguous();
     }
     if (p[0].defined() && p[1].defined()) p[1] = p[1].to(p[0].scalar_type());
-    if (at::GradMode::is_enabled() &&
-        (x.requires_grad() || (p[0].defined() && p[0].requires_grad()) ||
-         (p[1].defined() && p[1].requires_grad())))
+    if (recorded("nova_group_norm", {&x, &p[0], &p[1]}))
         return GroupNormFunction::apply(x, given(p[0]), given(p[1]), groups, eps, silu);
     Tensor stats;
     const at::AutoDispatchBelowADInplaceOrView below;
@@ -338,8 +350,7 @@ Tensor cross_attention(const Tensor& query, const Tensor& key, const Tensor& val
     }
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)D);
     const Tensor q = dense_rows(query), k = dense_rows(key), v = dense_rows(value);
-    if (at::GradMode::is_enabled() &&
-        (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    if (recorded("nova_cross_attention", {&q, &k, &v}))
         return AttentionFunction::apply(q, k, v, given(mask), scale);
     const at::AutoDispatchBelowADInplaceOrView below;
     return attention_forward(q, k, v, mask, scale, nullptr, nullptr);
