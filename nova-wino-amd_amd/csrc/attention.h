@@ -28,6 +28,11 @@ struct F16 {
     static __device__ __forceinline__ unsigned pack(float x, float y) {
         return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, h2));
     }
+    // two packed values times a power of two
+    static __device__ __forceinline__ unsigned scaled(unsigned v, float f) {
+        const _Float16 x = (_Float16)f;
+        return __builtin_bit_cast(unsigned, __builtin_bit_cast(h2, v) * h2{x, x});
+    }
     static __device__ __forceinline__ float lo(unsigned v) {
         return (float)__builtin_bit_cast(h2, v)[0];
     }
@@ -46,6 +51,7 @@ struct BF16 {
     static __device__ __forceinline__ unsigned pack(float x, float y) {
         return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, b2));
     }
+    static __device__ __forceinline__ unsigned scaled(unsigned v, float) { return v; }  // by 1
     static __device__ __forceinline__ float lo(unsigned v) {
         return __builtin_bit_cast(float, v << 16);
     }
@@ -381,6 +387,15 @@ __device__ __forceinline__ float max_wave(float x) {
     const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(u, 32));
     const float d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(u, 48));
     return fmaxf(fmaxf(a, b), fmaxf(c, d));
+}
+
+// x, -100 to 100, such that 2^x brings a float16 product's operands of up to
+// `largest` (>= 0) to between 2^7 and 2^8: eight bits of room above, for later
+// ones.
+__device__ __forceinline__ int half_range(float largest) {
+    int e;
+    (void)__builtin_frexpf(largest, &e);  // largest < 2^e
+    return largest > 0.0f ? min(max(8 - e, -100), 100) : 100;
 }
 
 // Place of a unit of the walk over query tiles: every tile of every query head

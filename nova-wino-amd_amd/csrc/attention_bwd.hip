@@ -63,10 +63,7 @@ struct Range {
     // so far have to be multiplied with.
     __device__ __forceinline__ float fit(float largest) {
         if (!(largest * f > 32768.0f || (f == 0.0f && largest > 0.0f))) return 1.0f;
-        int e;
-        (void)__builtin_frexpf(largest, &e);  // largest < 2^e
-        const int to = min(max(8 - e, -100), 100);
-        const float nf = __builtin_ldexpf(1.0f, to);
+        const float nf = __builtin_ldexpf(1.0f, half_range(largest));
         const float r = f == 0.0f ? 1.0f : nf / f;  // both powers of two
         f = nf;
         return r;

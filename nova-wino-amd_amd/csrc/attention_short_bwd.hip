@@ -16,9 +16,12 @@
 // workgroups that a CU's LDS holds. 64 heads of 40, 4096 rows, 77 keys: 50 us and
 // 4 us for the join of the workgroups' sums (dq, dk and dv over tiles: 80 us).
 //
-// float16: P enters times 2^10, ds times a power of two that the workgroup
-// shares; it moves, with the sums so far, only when a tile's largest value would
-// leave the type's range.
+// float16: P enters times 2^10, ds times a power of two: in dq one of the row's
+// own, in dk, whose sums run over the rows, one that the workgroup shares. That
+// one moves, with the sums so far, only when a tile's largest value would leave
+// the type's range: a dk's terms are off by up to 2^-32 of the largest ds that
+// the workgroup has met. (With the shared one in dq too, rows whose gradients
+// were 2^-20 of others' had errors of 1.6e-3, the type's own being 3e-4.)
 #include "attention.h"
 
 namespace nova {
@@ -140,7 +143,9 @@ __global__ __launch_bounds__(64 * NB, short_bwd_waves(DK, NB)) void attention_sh
                 s[kb][r] *= g[kb][r] - delta;
                 if (T::kHalf) top = fmaxf(top, fabsf(s[kb][r]));
             }
+        int up = 0;  // ds enters the row's own product, dq, times 2^up
         if (T::kHalf) {
+            up = half_range(max_halves(top));
             top = max_wave(top);
             if (lane == 0) tops[wave] = top;
         }
@@ -161,9 +166,7 @@ __global__ __launch_bounds__(64 * NB, short_bwd_waves(DK, NB)) void attention_sh
             top = __builtin_bit_cast(
                 float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
             if (top * f > 32768.0f || (f == 0.0f && top > 0.0f)) {
-                int e;
-                (void)__builtin_frexpf(top, &e);  // top < 2^e
-                const float to = __builtin_ldexpf(1.0f, min(max(8 - e, -100), 100));
+                const float to = __builtin_ldexpf(1.0f, half_range(top));
                 const float fix = f == 0.0f ? 1.0f : to / f;
                 f = to;
 #pragma unroll
@@ -171,18 +174,21 @@ __global__ __launch_bounds__(64 * NB, short_bwd_waves(DK, NB)) void attention_sh
             }
         }
         unsigned ds[NB][8];
+        const float fq = __builtin_ldexpf(1.0f, up);
 #pragma unroll
         for (int kb = 0; kb < NB; kb++)
 #pragma unroll
             for (int r = 0; r < 16; r += 2)
-                ds[kb][r / 2] = T::pack(s[kb][r] * f, s[kb][r + 1] * f);
+                ds[kb][r / 2] = T::pack(s[kb][r] * fq, s[kb][r + 1] * fq);
         lds_barrier();  // P is read
+        // from the row's power of two to the shared one: at most 2^8 times
+        const float to_all = __builtin_ldexpf(f, -up);
 #pragma unroll
         for (int kb = 0; kb < NB; kb++)
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
                 *reinterpret_cast<u2*>(prow + 32 * kb + acc_row(r)) =
-                    u2{ds[kb][r / 2], ds[kb][r / 2 + 1]};
+                    u2{T::scaled(ds[kb][r / 2], to_all), T::scaled(ds[kb][r / 2 + 1], to_all)};
         // dq of this wave's rows
         f16v acc[DV];
 #pragma unroll
@@ -201,7 +207,7 @@ __global__ __launch_bounds__(64 * NB, short_bwd_waves(DK, NB)) void attention_sh
             const int row = now.tile * kRows + mine, h = kvh * a.group + now.head, b = now.seq;
             if (row < a.Lq) {
                 float of = a.flip ? -a.scale : a.scale;
-                if (T::kHalf) of = f == 0.0f ? 0.0f : of / f * 0x1p-10f;
+                if (T::kHalf) of = __builtin_ldexpf(of, -up - 10);
                 uint16_t* p = a.dq + (((int64_t)b * a.Lq + row) * a.H + h) * a.D;
                 store_row<T, DV>(p, nullptr, acc, of, half, a.D);
             }

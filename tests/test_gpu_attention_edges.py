@@ -1,6 +1,7 @@
 """nova_cross_attention where it can go wrong beside its ordinary range: rows
-whose scores leave nothing at any scale. The definition in float64 and its
-tolerances are test_gpu_attention.py's."""
+whose scores leave nothing at any scale, and rows whose output gradients lie far
+apart. The definition in float64 and its tolerances are test_gpu_attention.py's
+where nothing else is said."""
 
 import pytest
 import torch
@@ -82,3 +83,46 @@ def test_scores_of_minus_infinity(Lq, Lk, H, D, scale):
     size = v.abs().amax(dim=(1, 3)).view(B, 1, H, 1).double()
     tol = 4 * 2.0 ** -8 * size.expand_as(got)
     _compare([got], [(want.double(), tol)], ["out"])
+
+
+def _query_gradient(q, k, v, go):
+    """float64, without a mask: grad_q and a bound on its error that holds each
+    row to its own values. ds is rounded to float16 (u), at a power of two that
+    leaves it off by 2^-32 of the row's largest where it is small; its float32
+    parts (see test_gpu_attention.py) are off by e; delta is their sum."""
+    D = q.shape[3]
+    u, e = 2.0 ** -11, 2.0 ** -24
+    Q, K, V, G = (t.double().transpose(1, 2).contiguous() for t in (q, k, v, go))
+    kt, vt = K.transpose(2, 3).contiguous(), V.transpose(2, 3).contiguous()
+    p = torch.softmax(torch.matmul(Q, kt) * D ** -0.5, 3)
+    top = (torch.matmul(Q.abs(), kt.abs()) * D ** -0.5).amax(3, keepdim=True)
+    rel = u + 4 * (D + 4) * e * top + 2.0 ** -19
+    dp, size = torch.matmul(G, vt), torch.matmul(G.abs(), vt.abs())
+    ds = p * (dp - (p * dp).sum(3, keepdim=True))
+    off = ds.abs() * rel + 2.0 ** -31 * ds.abs().amax(3, keepdim=True)
+    off = off + p * (D + 4) * e * (size + 2 * size.amax(3, keepdim=True))
+    dq = torch.matmul(ds, K) * D ** -0.5
+    tol = torch.matmul(off, K.abs()) * D ** -0.5 + u * dq.abs() + 2.0 ** -24
+    return dq.transpose(1, 2), tol.transpose(1, 2)
+
+
+@pytest.mark.parametrize("Lk,D", [(20, 64), (60, 40), (77, 40), (77, 64), (96, 160), (128, 80),
+                                  (129, 64)])
+def test_rows_with_gradients_far_apart(Lk, D):
+    """Each row's grad_q keeps the type's precision beside rows whose gradients
+    are 2^20 times as large, and beside rows that have none (float16)."""
+    g = torch.Generator(device=DEV).manual_seed(Lk)
+    B, H, Lq = 2, 2, 300
+    q, k, v = (_randn(g, B, n, H, D) for n in (Lq, Lk, Lk))
+    go = torch.randn(B, Lq, H, D, generator=g, device=DEV)
+    go[:, 2::3] = 0.0
+    for high, low in ((2.0 ** 10, 2.0 ** -10), (2.0 ** -4, 2.0 ** -4), (2.0 ** -20, 2.0 ** -20)):
+        gr = go.clone()
+        gr[:, ::3] *= high
+        gr[:, 1::3] *= low
+        gr = gr.half()
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        _nw().nova_cross_attention(*leaves).backward(gr)
+        _compare([leaves[0].grad], [_query_gradient(q, k, v, gr)], ["grad_q"])
+        assert not leaves[0].grad[:, 2::3].any()
+        assert all(t.grad.isfinite().all() for t in leaves)
