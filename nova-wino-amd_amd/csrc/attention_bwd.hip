@@ -469,13 +469,23 @@ static int64_t delta_bytes(const Attention& a) {
 
 // The short form: the keys that a workgroup's LDS holds; keys that sequences
 // share under a mask may hold anything where another sequence keeps them, which
-// the long form's walks tell apart. Few rows (a few hundred) take the long form
-// with p and ds as two terms each: the roundings of some dozen large p do not
-// average out in a gradient, and its time is the launches' either way (one head
-// of 64, 77 keys, forward and backward: 513 rows 26 us, 512 rows 32). The short
-// form against the tiles, backward alone, us: 64 heads of 40, 4096 rows, 77 keys
-// 50 | 80; 64 heads of 80, 1024 rows, 128 keys 41 | 54; 16 heads of 160, 4096
-// rows, 96 keys 61 | 99.
+// the long form's walks tell apart. The short form against the tiles, backward
+// alone, us: 64 heads of 40, 4096 rows, 77 keys 50 | 80; 64 heads of 80, 1024 rows,
+// 128 keys 41 | 54; 16 heads of 160, 4096 rows, 96 keys 84 | 96 in bfloat16. In
+// float16, where both keep some of that size's values in scratch, 114 | 108; 64
+// heads of 160, 1024 rows, 77 keys 110 | 105, 60 keys 77 | 85, 8 heads 39 | 54. The
+// forward is 6 us faster without the rest that it writes for the tiles, so that
+// those steps are even: 133 | 134, and 137 | 137 with 96 keys.
+//
+// Few rows in the whole call take the long form with p and ds as two terms each.
+// One rounding of p and ds makes a gradient's error 1.42 times that of its own
+// last rounding for any number of rows; two terms, 1.04. What few rows change is
+// the spread: few p and ds hold most of a gradient, and their luck decides.
+// Largest of 24 calls, one term | two: 1 row 2.4 | 1.0, 64 rows 1.64 | 1.07, 512
+// rows 1.53 | 1.06, 1024 rows 1.50. The price, forward and backward, us, for 512
+// rows of 64 channels: 77 keys, one head 23 | 32, 64 heads 15 | 27, 512 heads 19 |
+// 42; 333 keys, one head 43 | 46; 1500 keys, 64 heads 100 | 112 (a step's host part
+// is some 65 outside of a graph).
 static bool few_rows(const Attention& a) { return (int64_t)a.B * a.H * a.Lq <= 512; }
 
 static bool short_bwd(const Attention& a) {
