@@ -134,8 +134,8 @@ Norm norm_of(const Tensor& x, int64_t groups, const Tensor& weight, const Tensor
     return n;
 }
 
-// y; *stats: mean and 1 / standard deviation, [2][B][G], in front of the
-// workspace.
+// y. stats: gets mean and 1 / standard deviation, [2][B][G], for a backward; or
+// null, and they share one allocation with the workspace.
 Tensor norm_forward(const Norm& n, Tensor* stats) {
     const c10::DeviceGuard guard(n.x.device());
     const nova_group_norm_t a = n.args();
@@ -143,11 +143,17 @@ Tensor norm_forward(const Norm& n, Tensor* stats) {
     if (ws < 0) check("group_norm");
     const int64_t count = (int64_t)a.batch * a.groups;
     const int64_t front = (2 * count + 3) / 4 * 4;  // the workspace starts on 16 bytes
-    *stats = at::empty({front + (ws + 3) / 4}, n.x.options().dtype(at::kFloat),
-                       at::MemoryFormat::Contiguous);
+    Tensor both, work;
+    both = at::empty({front + (stats ? 0 : (ws + 3) / 4)}, n.x.options().dtype(at::kFloat),
+                     at::MemoryFormat::Contiguous);
+    if (stats) {
+        *stats = both;
+        if (ws > 0) work = scratch(n.x, ws, "group_norm");
+    }
     Tensor y = at::empty_like(n.x, n.x.options(), n.format);
-    float* s = stats->mutable_data_ptr<float>();
-    nova_group_norm(&a, y.mutable_data_ptr(), s, s + count, s + front, ws, stream_of(n.x));
+    float* s = both.mutable_data_ptr<float>();
+    void* w = work.defined() ? work.mutable_data_ptr() : s + front;
+    nova_group_norm(&a, y.mutable_data_ptr(), s, s + count, w, ws, stream_of(n.x));
     check("group_norm");
     return y;
 }
@@ -223,9 +229,8 @@ Tensor group_norm(const Tensor& x, int64_t groups, const std::optional<Tensor>& 
     if (p[0].defined() && p[1].defined()) p[1] = p[1].to(p[0].scalar_type());
     if (recorded("nova_group_norm", {&x, &p[0], &p[1]}))
         return GroupNormFunction::apply(x, given(p[0]), given(p[1]), groups, eps, silu);
-    Tensor stats;
     const at::AutoDispatchBelowADInplaceOrView below;
-    return norm_forward(norm_of(x, groups, p[0], p[1], eps, silu), &stats);
+    return norm_forward(norm_of(x, groups, p[0], p[1], eps, silu), nullptr);
 }
 
 // ---- attention ----------------------------------------------------------------

@@ -1,6 +1,8 @@
-"""nova_group_norm with more groups than a workgroup of its layout's width has
-threads: three to seven channels a group above 2048 channels, channels-last. The
-definition in float64 and its tolerances are test_gpu_group_norm.py's."""
+"""nova_group_norm at sizes beyond the ordinary: more groups than a workgroup of
+its layout's width has threads (three to seven channels a group above 2048
+channels, channels-last), more elements than the element-by-element form's
+grid, and what a training step keeps in memory. The definition in float64 and its
+tolerances are test_gpu_group_norm.py's."""
 
 import pytest
 import torch
@@ -47,3 +49,18 @@ def test_more_elements_than_the_plain_grid():
         nova_group_norm(one, 32, activation="silu").backward(gy[i:i + 1])
         assert torch.equal(one.grad, both.grad[i:i + 1])
         assert one.grad.count_nonzero() > 0.9 * one.numel()
+
+
+@pytest.mark.parametrize("shape", [(64, 1024, 32, 16, 16), (4, 320, 32, 64, 64)])
+@pytest.mark.parametrize("nhwc", [True, False])
+def test_memory_kept_for_the_backward(shape, nhwc):
+    """The statistics, 8 bytes for each image and group, and no workspace."""
+    from nova_winograd import nova_group_norm
+
+    B, C, G, H, W = shape
+    x = _case(B, C, H, W, torch.float16, nhwc)[0].requires_grad_()
+    nova_group_norm(x, G)
+    before = torch.cuda.memory_allocated()
+    y = nova_group_norm(x, G)
+    kept = torch.cuda.memory_allocated() - before - 2 * y.numel()
+    assert kept <= 8 * B * G + 2 * 512  # the allocator's blocks
