@@ -39,7 +39,6 @@ struct F16 {
     static __device__ __forceinline__ float hi(unsigned v) {
         return (float)__builtin_bit_cast(h2, v)[1];
     }
-    static constexpr unsigned kSigns = 0x80008000u;
 };
 
 struct BF16 {
@@ -58,7 +57,6 @@ struct BF16 {
     static __device__ __forceinline__ float hi(unsigned v) {
         return __builtin_bit_cast(float, v & 0xffff0000u);
     }
-    static constexpr unsigned kSigns = 0x80008000u;
 };
 
 // Keys per tile of the kernels that walk the keys, and tiles whose masks one

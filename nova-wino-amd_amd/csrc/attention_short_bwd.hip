@@ -44,7 +44,7 @@ struct ShortBwdArgs {
 };
 
 // Waves per SIMD that the registers are cut for: two where nothing spills.
-constexpr int short_bwd_waves(int DK, int NB) { return NB <= 3 && DK <= (NB == 2 ? 5 : 4) ? 2 : 1; }
+constexpr int short_bwd_waves(int DK, int NB) { return NB <= 3 && DK <= 4 ? 2 : 1; }
 
 template <typename T, int DK, int NB>
 __global__ __launch_bounds__(64 * NB, short_bwd_waves(DK, NB)) void attention_short_bwd_kernel(
