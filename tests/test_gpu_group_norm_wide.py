@@ -51,10 +51,11 @@ def test_more_elements_than_the_plain_grid():
         assert one.grad.count_nonzero() > 0.9 * one.numel()
 
 
-@pytest.mark.parametrize("shape", [(64, 1024, 32, 16, 16), (4, 320, 32, 64, 64)])
+@pytest.mark.parametrize("shape", [(4, 10240, 32, 3, 3), (4, 320, 32, 64, 64), (64, 960, 32, 5, 3)])
 @pytest.mark.parametrize("nhwc", [True, False])
 def test_memory_kept_for_the_backward(shape, nhwc):
-    """The statistics, 8 bytes for each image and group, and no workspace."""
+    """The statistics, 8 bytes for each image and group, and of the workspace at
+    most 1/16 of the input."""
     from nova_winograd import nova_group_norm
 
     B, C, G, H, W = shape
@@ -63,4 +64,4 @@ def test_memory_kept_for_the_backward(shape, nhwc):
     before = torch.cuda.memory_allocated()
     y = nova_group_norm(x, G)
     kept = torch.cuda.memory_allocated() - before - 2 * y.numel()
-    assert kept <= 8 * B * G + 2 * 512  # the allocator's blocks
+    assert kept <= 8 * B * G + x.numel() // 8 + 2 * 512  # the allocator's blocks
