@@ -31,9 +31,9 @@ def nova_cross_attention(query, key, value, key_mask=None, scale=None):
 
     Returns a dense [B, Lq, H, D] tensor of the query's type. Scores, sums and
     outputs are accumulated in float32, the probabilities rounded to the
-    inputs' type for their product. Differentiable (once) with respect to
-    query, key and value. Runs on PyTorch's current stream; results do not
-    change from call to call.
+    inputs' type for their product. Differentiable (once, in reverse mode) with
+    respect to query, key and value. Runs on PyTorch's current stream; results
+    do not change from call to call.
     """
     return native().cross_attention(query, key, value, key_mask, scale)
 

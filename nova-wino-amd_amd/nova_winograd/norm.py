@@ -36,8 +36,9 @@ def nova_group_norm(input, num_groups, weight=None, bias=None, eps=1e-5, activat
         activation: None or "silu".
 
     Returns a tensor of the input's shape, type and layout. Statistics are
-    float32; every value is rounded once. Differentiable (once) with respect to
-    input, weight and bias. Runs on PyTorch's current stream.
+    float32; every value is rounded once. Differentiable (once, in reverse
+    mode) with respect to input, weight and bias. Runs on PyTorch's current
+    stream.
     """
     silu = _silu("nova_group_norm", activation)
     if not isinstance(num_groups, int):
